@@ -78,6 +78,9 @@ __device__ inline int divide_lanes(int a, int b, bool small) {
   return q + ((q + 1) * b <= a);
 }
 
+// The first key that position p sees; p may lie below 0 and the window be as large as an int holds.
+__device__ inline int first_key(int p, int window) { return window && p >= window ? p - window + 1 : 0; }
+
 // A request as a kernel walks it: row tiles of RPT rows, for each kv head an item of nt steps from tile0;
 // an item is worth a unit for every PER steps and COST more. A launch's units are below 2^31 (its host side
 // sees to that).
@@ -95,7 +98,7 @@ __device__ inline Req request(const Attend &a, int begin, int end, int len) {
   const int64_t room = (int64_t)a.cols << a.shift;
   q.len = (int)min((int64_t)max(len, 0), room);
   const int p0 = q.len - q.n;  // the first token's position, below 0 where it sees nothing
-  const int lo = a.window ? max(0, p0 - a.window + 1) : 0;
+  const int lo = first_key(p0, a.window);
   q.tile0 = min(lo, max(q.len - 1, 0)) / kStep;
   q.nt = max(q.len - 1, 0) / kStep - q.tile0 + 1;  // one step, all of it masked, where there is no key
   q.row_tiles = ((int64_t)q.n * (a.heads / a.heads_kv) + RPT - 1) / RPT;

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     auto token_of = [&](int rr) { return rq.n == 1 ? 0 : divide(rr, group); };
     const int p_last = rq.len - rq.n + token_of(row0 + rows - 1);   // of the tile's rows
     const int p_first = rq.len - rq.n + token_of(row0);
-    const int first_last = a.window ? max(0, p_last - a.window + 1) : 0;
+    const int first_last = first_key(p_last, a.window);
     const int32_t *table = a.table + (size_t)r * a.cols;
 
     // ---- page ids of this wave's next 16 steps, a lane for each granule
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
     auto pair_of = [&](int i) { return min(64 * i + lane, D / 2 - 1); };
     const int my_row = row0 + min(row, rows - 1), my_token = divide_lanes(my_row, group, rows_all < 1 << 22);
     const int pos = row < rows ? rq.len - rq.n + my_token : INT32_MAX;
-    const int first = a.window && row < rows ? max(0, pos - a.window + 1) : 0;
+    const int first = row < rows ? first_key(pos, a.window) : 0;
     const int64_t my_q = (int64_t)(rq.token0 + my_token) * a.ldq + (kvh * group + my_row - my_token * group) * D;
     float x[RW][PL][2];
 #pragma unroll

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     const int tile = item / a.heads_kv, rt = rq.row_tiles - 1 - tile, kvh = item - tile * a.heads_kv;
     const int row0 = rt * kRows, rows = min(kRows, rq.n * group - row0);
     const int p_first = rq.len - rq.n + row0 / group, p_last = rq.len - rq.n + (row0 + rows - 1) / group;
-    const int first_last = a.window ? max(0, p_last - a.window + 1) : 0, lowest = a.window ? max(0, p_first - a.window + 1) : 0;
+    const int first_last = first_key(p_last, a.window), lowest = first_key(p_first, a.window);
     // the steps of this part that some row of the tile sees
     t0 = max(t0, lowest / kStep - rq.tile0);
     t1 = p_last < 0 ? t0 : min(t1, p_last / kStep - rq.tile0 + 1);
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       if (t + 2 < t1) load(t + 2, page, P);
       if (!whole) {
         const Row q = my_row();
-        const int pos = q.rho < rows ? rq.len - rq.n + q.token : INT32_MAX, first = a.window && q.rho < rows ? max(0, pos - a.window + 1) : 0;
+        const int pos = q.rho < rows ? rq.len - rq.n + q.token : INT32_MAX, first = q.rho < rows ? first_key(pos, a.window) : 0;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           const uint32_t bad = bad_keys[t & 1][2 * kt + h];
