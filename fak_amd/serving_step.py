@@ -11,6 +11,7 @@ and embeddings are random: the answers mean nothing, the log probabilities and t
 from __future__ import annotations
 
 import argparse
+import contextlib
 import ctypes as C
 import time
 
@@ -25,7 +26,11 @@ class Buffer:
     def __init__(self, nbytes: int, host: np.ndarray = None):
         self.ptr = fakhip.alloc_call("fhip_malloc", max(nbytes, 16))
         if host is not None:
-            self.put(host)
+            try:
+                self.put(host)
+            except Exception:
+                self.free()
+                raise
 
     def put(self, a: np.ndarray) -> None:
         a = np.ascontiguousarray(a)
@@ -65,19 +70,28 @@ class Server:
         self.vocab, self.page, self.window, self.top = vocab, page, window, top
         self.cols = -(-positions // page)
         self.pages = requests * self.cols
-        size = fakhip.load().fhip_kv4_cache_bytes(self.pages, page, heads_kv, dim)
         self.held = []
+        try:
+            self.fill(layers, seed)
+        except Exception:
+            self.close()
+            raise
+
+    def fill(self, layers, seed) -> None:
+        """Weights, caches and the pages' bookkeeping."""
+        size = fakhip.load().fhip_kv4_cache_bytes(self.pages, self.page, self.HK, self.D)
         self.layers = []
         for i in range(layers):
             w = [self.weight(out, in_, seed + 7 * i + j)
-                 for j, (out, in_) in enumerate([(heads * dim, hidden), (heads_kv * dim, hidden), (heads_kv * dim, hidden), (hidden, heads * dim)])]
+                 for j, (out, in_) in enumerate([(self.H * self.D, self.hidden), (self.HK * self.D, self.hidden), (self.HK * self.D, self.hidden),
+                                                 (self.hidden, self.H * self.D)])]
             self.layers.append((w, self.hold(Buffer(size))))
-        self.head = self.weight(vocab, hidden, seed + 1000)
+        self.head = self.weight(self.vocab, self.hidden, seed + 1000)
         self.free_list = self.hold(ints(np.random.default_rng(seed).permutation(self.pages)))
-        self.table = self.hold(ints(np.full((requests, self.cols), -1)))
-        self.lens, self.lens_next = self.hold(ints(np.zeros(requests))), self.hold(ints(np.zeros(requests)))
+        self.table = self.hold(ints(np.full((self.R, self.cols), -1)))
+        self.lens, self.lens_next = self.hold(ints(np.zeros(self.R))), self.hold(ints(np.zeros(self.R)))
         self.taken, self.taken_next = self.hold(ints([0, 0])), self.hold(ints([0, 0]))
-        self.start = self.hold(ints(np.zeros(requests + 1)))
+        self.start = self.hold(ints(np.zeros(self.R + 1)))
 
     def hold(self, b: Buffer) -> Buffer:
         self.held.append(b)
@@ -97,42 +111,46 @@ class Server:
         """tokens[r]: the request's new token ids (none: it waits). Returns for each request with any the next
         id, and the given tokens' log probabilities where the batch knows them: token i + 1 of a request after
         its token i; and the entropy after its last."""
+        with contextlib.ExitStack() as stack:
+            return self.run(tokens, stack)
+
+    def run(self, tokens, stack):
+        """A step whose buffers are the stack's."""
+        def own(b: Buffer) -> Buffer:
+            stack.callback(b.free)
+            return b
+
         flat = np.concatenate([np.asarray(t, np.int64) for t in tokens]) if any(len(t) for t in tokens) else np.zeros(0, np.int64)
         T, R, H, HK, D = len(flat), self.R, self.H, self.HK, self.D
         counts = [len(t) for t in tokens]
-        fresh, slots, pos = ints(counts), ints(np.zeros(T)), ints(np.zeros(T))
-        q, k, v, o = (Buffer(T * n * 4) for n in (H * D, HK * D, HK * D, H * D))
-        x_dev, y_dev, logits = Buffer(T * self.hidden * 4), Buffer(T * self.hidden * 4), Buffer(T * self.vocab * 4)
-        following = np.concatenate([np.append(np.asarray(t[1:], np.int32), np.int32(-1)) if len(t) else np.zeros(0, np.int32) for t in tokens])
-        given, logp, entropy, tl, ti = ints(following), Buffer(T * 4), Buffer(T * 4), Buffer(T * self.top * 4), Buffer(T * self.top * 4)
-        try:
-            fakhip.call("fhip_kv_slots_i32", self.lens.ptr, fresh.ptr, self.free_list.ptr, self.taken.ptr, self.table.ptr, slots.ptr, pos.ptr,
-                        self.start.ptr, self.lens_next.ptr, self.taken_next.ptr, R, T, self.cols, self.pages, self.page)
-            self.lens, self.lens_next = self.lens_next, self.lens
-            self.taken, self.taken_next = self.taken_next, self.taken
-            where = pos.get(T, np.int32)
-            if self.taken.get(2, np.int32)[1]:
-                raise RuntimeError("requests past the pages or the table")
-            x = np.stack([np.random.default_rng(int(t)).standard_normal(self.hidden).astype(np.float32) for t in flat])
-            for (wq, wk, wv, wo), cache in self.layers:
-                x_dev.put(unit_rows(x))
-                w = (C.c_void_p * 3)(wq, wk, wv)
-                y = (C.c_void_p * 3)(q.ptr, k.ptr, v.ptr)
-                fakhip.call("fhip_q4k_matmul_group_f32", w, y, (C.c_int * 3)(H * D, HK * D, HK * D), 3, x_dev.ptr, self.hidden, T)
-                q.put(rotate(unit_rows(q.get((T, H, D))), where))
-                k.put(rotate(unit_rows(k.get((T, HK, D))), where))
-                fakhip.call("fhip_kv4_append_f32", cache.ptr, k.ptr, v.ptr, slots.ptr, T, HK, D, self.pages, self.page, HK * D, HK * D)
-                fakhip.call("fhip_kv4_attention_f32", cache.ptr, q.ptr, o.ptr, self.start.ptr, self.lens.ptr, self.table.ptr, R, T, max(counts),
-                            H, HK, D, self.pages, self.page, self.cols, H * D, self.window, D ** -0.5)
-                fakhip.call("fhip_q4k_matmul_f32", wo, o.ptr, y_dev.ptr, self.hidden, H * D, T)
-                x = x + unit_rows(y_dev.get((T, self.hidden)))
-            x_dev.put(unit_rows(x) * np.float32(0.01))
-            fakhip.call("fhip_q4k_matmul_f32", self.head, x_dev.ptr, logits.ptr, self.vocab, self.hidden, T)
-            fakhip.call("fhip_logprobs_f32", logits.ptr, given.ptr, logp.ptr, entropy.ptr, tl.ptr, ti.ptr, T, self.vocab, self.vocab, self.top)
-            logp, entropy, ti = logp.get(T), entropy.get(T), ti.get((T, self.top), np.int32)
-        finally:
-            for b in (fresh, slots, pos, q, k, v, o, x_dev, y_dev, logits, given, *(b for b in (logp, entropy, tl, ti) if isinstance(b, Buffer))):
-                b.free()
+        fresh, slots, pos = own(ints(counts)), own(ints(np.zeros(T))), own(ints(np.zeros(T)))
+        q, k, v, o, x_dev, y_dev, logits, logp_dev, entropy_dev, tl_dev, ti_dev = (
+            own(Buffer(T * n * 4)) for n in (H * D, HK * D, HK * D, H * D, self.hidden, self.hidden, self.vocab, 1, 1, self.top, self.top))
+        given = own(ints(np.concatenate([np.append(np.asarray(t[1:], np.int32), np.int32(-1)) if len(t) else np.zeros(0, np.int32) for t in tokens])))
+        fakhip.call("fhip_kv_slots_i32", self.lens.ptr, fresh.ptr, self.free_list.ptr, self.taken.ptr, self.table.ptr, slots.ptr, pos.ptr,
+                    self.start.ptr, self.lens_next.ptr, self.taken_next.ptr, R, T, self.cols, self.pages, self.page)
+        self.lens, self.lens_next = self.lens_next, self.lens
+        self.taken, self.taken_next = self.taken_next, self.taken
+        where = pos.get(T, np.int32)
+        if self.taken.get(2, np.int32)[1]:
+            raise RuntimeError("requests past the pages or the table")
+        x = np.stack([np.random.default_rng(int(t)).standard_normal(self.hidden).astype(np.float32) for t in flat])
+        for (wq, wk, wv, wo), cache in self.layers:
+            x_dev.put(unit_rows(x))
+            w = (C.c_void_p * 3)(wq, wk, wv)
+            y = (C.c_void_p * 3)(q.ptr, k.ptr, v.ptr)
+            fakhip.call("fhip_q4k_matmul_group_f32", w, y, (C.c_int * 3)(H * D, HK * D, HK * D), 3, x_dev.ptr, self.hidden, T)
+            q.put(rotate(unit_rows(q.get((T, H, D))), where))
+            k.put(rotate(unit_rows(k.get((T, HK, D))), where))
+            fakhip.call("fhip_kv4_append_f32", cache.ptr, k.ptr, v.ptr, slots.ptr, T, HK, D, self.pages, self.page, HK * D, HK * D)
+            fakhip.call("fhip_kv4_attention_f32", cache.ptr, q.ptr, o.ptr, self.start.ptr, self.lens.ptr, self.table.ptr, R, T, max(counts),
+                        H, HK, D, self.pages, self.page, self.cols, H * D, self.window, D ** -0.5)
+            fakhip.call("fhip_q4k_matmul_f32", wo, o.ptr, y_dev.ptr, self.hidden, H * D, T)
+            x = x + unit_rows(y_dev.get((T, self.hidden)))
+        x_dev.put(unit_rows(x) * np.float32(0.01))
+        fakhip.call("fhip_q4k_matmul_f32", self.head, x_dev.ptr, logits.ptr, self.vocab, self.hidden, T)
+        fakhip.call("fhip_logprobs_f32", logits.ptr, given.ptr, logp_dev.ptr, entropy_dev.ptr, tl_dev.ptr, ti_dev.ptr, T, self.vocab, self.vocab, self.top)
+        logp, entropy, ti = logp_dev.get(T), entropy_dev.get(T), ti_dev.get((T, self.top), np.int32)
         out, at = [], 0
         for n in counts:
             out.append((int(ti[at + n - 1, 0]), logp[at:at + n - 1], float(entropy[at + n - 1])) if n else None)
