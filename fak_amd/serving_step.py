@@ -110,7 +110,10 @@ class Server:
     def step(self, tokens):
         """tokens[r]: the request's new token ids (none: it waits). Returns for each request with any the next
         id, and the given tokens' log probabilities where the batch knows them: token i + 1 of a request after
-        its token i; and the entropy after its last."""
+        its token i; and the entropy after its last. A step that finds no room for a request raises and leaves
+        lengths and pages as they were."""
+        if not any(len(t) for t in tokens):
+            return [None] * self.R
         with contextlib.ExitStack() as stack:
             return self.run(tokens, stack)
 
@@ -120,7 +123,7 @@ class Server:
             stack.callback(b.free)
             return b
 
-        flat = np.concatenate([np.asarray(t, np.int64) for t in tokens]) if any(len(t) for t in tokens) else np.zeros(0, np.int64)
+        flat = np.concatenate([np.asarray(t, np.int64) for t in tokens])
         T, R, H, HK, D = len(flat), self.R, self.H, self.HK, self.D
         counts = [len(t) for t in tokens]
         fresh, slots, pos = own(ints(counts)), own(ints(np.zeros(T))), own(ints(np.zeros(T)))
@@ -129,11 +132,11 @@ class Server:
         given = own(ints(np.concatenate([np.append(np.asarray(t[1:], np.int32), np.int32(-1)) if len(t) else np.zeros(0, np.int32) for t in tokens])))
         fakhip.call("fhip_kv_slots_i32", self.lens.ptr, fresh.ptr, self.free_list.ptr, self.taken.ptr, self.table.ptr, slots.ptr, pos.ptr,
                     self.start.ptr, self.lens_next.ptr, self.taken_next.ptr, R, T, self.cols, self.pages, self.page)
+        where = pos.get(T, np.int32)
+        if self.taken_next.get(2, np.int32)[1]:  # nothing is written yet, and the pages named in the table are named anew
+            raise RuntimeError("requests past the pages or the table")
         self.lens, self.lens_next = self.lens_next, self.lens
         self.taken, self.taken_next = self.taken_next, self.taken
-        where = pos.get(T, np.int32)
-        if self.taken.get(2, np.int32)[1]:
-            raise RuntimeError("requests past the pages or the table")
         x = np.stack([np.random.default_rng(int(t)).standard_normal(self.hidden).astype(np.float32) for t in flat])
         for (wq, wk, wv, wo), cache in self.layers:
             x_dev.put(unit_rows(x))

@@ -92,3 +92,26 @@ def test_a_server_that_cannot_be_built_leaves_nothing_behind(library):
         with pytest.raises(MemoryError):
             server()
         assert not library.live
+
+
+def test_all_requests_wait(library):
+    s = server()
+    s.step([[1, 2], [3], []])
+    state, before = held(s, library), set(library.live)
+    assert s.step([[], [], []]) == [None] * 3
+    assert held(s, library) == state and set(library.live) == before
+    assert s.step([[4], [], [5]])[1] is None and held(s, library)[0] == [3, 1, 1]
+
+
+def test_a_refused_step_changes_nothing(library):
+    """A request past its table's row: the others' lengths and pages stay too, as no key was written."""
+    s = server()
+    s.step([[1] * 20, [2], [3]])
+    state, before = held(s, library), set(library.live)
+    library.calls.clear()
+    with pytest.raises(RuntimeError):
+        s.step([[4], [5] * 64, [6]])
+    assert held(s, library) == state and set(library.live) == before
+    assert "fhip_kv4_append_f32" not in library.calls
+    s.step([[4], [5], [6]])
+    assert held(s, library) == ([21, 2, 2], 4)
