@@ -81,6 +81,12 @@ __device__ inline int divide_lanes(int a, int b, bool small) {
 // The first key that position p sees; p may lie below 0 and the window be as large as an int holds.
 __device__ inline int first_key(int p, int window) { return window && p >= window ? p - window + 1 : 0; }
 
+// Bits lo to hi of 64, which may lie outside.
+__device__ inline uint64_t keys_between(int lo, int hi) {
+  lo = max(lo, 0), hi = min(hi, 63);
+  return lo <= hi ? (~0ull >> (63 - hi)) & (~0ull << lo) : 0;
+}
+
 // A request as a kernel walks it: row tiles of RPT rows, for each kv head an item of nt steps from tile0;
 // an item is worth a unit for every PER steps and COST more. A launch's units are below 2^31 (its host side
 // sees to that).

@@ -336,21 +336,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
         for (int b = 0; b < NB; ++b) ksc[t4][b] = sc[b];
       }
       __builtin_amdgcn_sched_barrier(0);
-      uint64_t bad = 0;
       if (!whole) {
-        // Keys that some row does not see. What they hold must not reach it: a V scale that no written
-        // block has (NaN, or bytes left by someone else) counts as 0, and a row that does see the key
-        // gets its NaN by the score.
+        // Keys that some row does not see. What they hold must not reach it: a V scale that no written block has
+        // (NaN, or bytes left by someone else) counts as 0, and a row that does see the key gets the NaN in the
+        // block's sums, where the product would have put it.
         _Float16 *s = reinterpret_cast<_Float16 *>(buf);
-        bool any = false;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const float v = (float)s[san_at + 16 * b + kv4_v_place(col)];
-          const bool odd = !(fabsf(v) <= kMaxScale);
-          any |= odd;
-          if (odd) s[san_at + 16 * b + kv4_v_place(col)] = (_Float16)0.f;
+          const bool odd = !(fabsf((float)s[san_at + 16 * b + kv4_v_place(col)]) <= kMaxScale);
+          if (const uint64_t bad = __ballot(odd)) {  // bit j: key k0 + j
+            if (odd) s[san_at + 16 * b + kv4_v_place(col)] = (_Float16)0.f;
+            const float taint = bad & keys_between(first - k0, pos - k0) ? __builtin_nanf("") : 0.f;
+            o[2 * b] += taint, o[2 * b + 1] += taint;
+          }
         }
-        bad = __ballot(any);
         asm volatile("" ::: "memory");  // the words just written are read below as another type
       }
       f32x4 s[4];
@@ -390,7 +389,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = k0 + 16 * g + 4 * t4 + i;
-            if ((bad >> (16 * g + 4 * t4 + i)) & 1) x[t4][i] = __builtin_nanf("");
             if (key < first || key > pos) x[t4][i] = -__builtin_inff();
           }
       }

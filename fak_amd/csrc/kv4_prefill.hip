@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   constexpr int KU = D / 8 + 1, VU = 9;                // 16-byte units of a K row, a V column (a pad each)
   __shared__ u32x4 P0[kWaves * GW / 4], P1[kWaves * GW / 4];  // packed granules, a wave's own
   __shared__ u32x4 KF[64 * KU], VF[D * VU];
-  __shared__ uint32_t bad_keys[2][kWaves];  // of odd and even steps
+  __shared__ __align__(8) uint16_t bad_keys[2][NB][kWaves];  // of odd and even steps, by block and granule
   __shared__ int scan_i[kWaves], scan_u[kWaves], found_before, found_r;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31, l16 = lane & 15, q4 = lane >> 4;
@@ -258,19 +258,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       const bool whole = k0 >= first_last && k0 + kStep - 1 <= p_first;
       landed();
       const int page = page_of(min(t + 2, t1 - 1));
-      if (!whole) {  // as in kv4_attention.hip: what some row does not see counts as 0, or NaN by the score
+      if (!whole) {  // as in kv4_attention.hip: what some row does not see counts as 0, or NaN by the sums
         _Float16 *s = reinterpret_cast<_Float16 *>(P);
         const uint32_t psan = in_reg(2 * (wave * GW + 17 * D / 4) + kv4_v_place(threadIdx.x & 15));
-        bool any = false;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const float v = (float)s[psan + 16 * b];
-          const bool odd = !(fabsf(v) <= kMaxScale);
-          any |= odd;
+          const bool odd = !(fabsf((float)s[psan + 16 * b]) <= kMaxScale);
           if (odd) s[psan + 16 * b] = (_Float16)0.f;
+          const uint64_t bad = __ballot(odd);
+          if (lane == 0) bad_keys[t & 1][b][wave] = (uint16_t)bad;
         }
-        const uint64_t bad = __ballot(any);
-        if (lane == 0) bad_keys[t & 1][wave] = (uint32_t)bad & 0xFFFFu;
         asm volatile("" ::: "memory");
       }
       f32x16 s[2];
@@ -310,15 +307,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         const Row q = my_row();
         const int pos = q.rho < rows ? rq.len - rq.n + q.token : INT32_MAX, first = q.rho < rows ? first_key(pos, a.window) : 0;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          const uint32_t bad = bad_keys[t & 1][2 * kt + h];
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int key = k0 + 32 * kt + 16 * h + i;
-            if ((bad >> i) & 1) s[kt][i] = __builtin_nanf("");
             if (key < first || key > pos) s[kt][i] = -__builtin_inff();
           }
-        }
+        const uint64_t seen = keys_between(first - k0, pos - k0);
+#pragma unroll
+        for (int d = 0; d < NB; ++d)
+          if (const uint64_t bad = *reinterpret_cast<const uint64_t *>(bad_keys[t & 1][d]); __any(bad != 0)) o[d] += bad & seen ? __builtin_nanf("") : 0.f;
       }
       float mx = -__builtin_inff();
 #pragma unroll

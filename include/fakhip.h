@@ -317,8 +317,9 @@ int fhip_kv4_read_f32(float *dK, float *dV, const void *dCache, const int32_t *d
  * exact values: within 1e-5 of the formula in the 2-norm; a weight below 2^-38 of its row's largest counts as
  * zero. scale is in (0, 1e37]. requests up to 65535. The steps of 64 keys that a table row allows, for each kv head
  * and each 8 rows (tokens times heads / heads_kv; 16 or 128 rows where there are more), stay below about 2^31
- * for a batch's tokens, or the call is refused as too many. NaN keys, values or queries make the outputs
- * that see them NaN; what lies behind a request's length is never seen. No counterpart in the
+ * for a batch's tokens, or the call is refused as too many. A NaN in a query makes its head's outputs
+ * NaN, one in a key those of the rows that see it, one in a block of 32 values these 32 dimensions of them (an
+ * infinity the same); what lies behind a request's length is never seen. No counterpart in the
  * reference's device path (attention there reads an f32 cache, internal/compute/cuda_kernels.cu). */
 int fhip_kv4_attention_f32(const void *dCache, const float *dQ, float *dOut, const int32_t *dStart,
                            const int32_t *dLens, const int32_t *dTable, int requests, int tokens, int max_new,
