@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   constexpr int KU = D / 8 + 1, VU = 9;                // 16-byte units of a K row, a V column (a pad each)
   __shared__ u32x4 P0[kWaves * GW / 4], P1[kWaves * GW / 4];  // packed granules, a wave's own
   __shared__ u32x4 KF[64 * KU], VF[D * VU];
-  __shared__ __align__(8) uint16_t bad_keys[2][NB][kWaves];  // of odd and even steps, by block and granule
+  __shared__ uint8_t bad_blocks[2][kStep];  // of each key of odd and even steps: a bit for each block
   __shared__ int scan_i[kWaves], scan_u[kWaves], found_before, found_r;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31, l16 = lane & 15, q4 = lane >> 4;
@@ -177,6 +177,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     }
     f32x16 o[NB];
     float m = -__builtin_inff(), l = 0.f;
+    uint32_t taint = 0;  // blocks of 32 dimensions that are NaN
 #pragma unroll
     for (int d = 0; d < NB; ++d)
 #pragma unroll
@@ -261,13 +262,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       if (!whole) {  // as in kv4_attention.hip: what some row does not see counts as 0, or NaN by the sums
         _Float16 *s = reinterpret_cast<_Float16 *>(P);
         const uint32_t psan = in_reg(2 * (wave * GW + 17 * D / 4) + kv4_v_place(threadIdx.x & 15));
+        uint32_t bad = 0;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const bool odd = !(fabsf((float)s[psan + 16 * b]) <= kMaxScale);
-          if (odd) s[psan + 16 * b] = (_Float16)0.f;
-          const uint64_t bad = __ballot(odd);
-          if (lane == 0) bad_keys[t & 1][b][wave] = (uint16_t)bad;
+        for (int b = 0; b < NB; ++b) {  // (four lanes to a token, with the same; masks of lanes would need scalar registers)
+          const _Float16 v = s[psan + 16 * b];
+          const bool odd = !(fabsf((float)v) <= kMaxScale);
+          s[psan + 16 * b] = odd ? (_Float16)0.f : v;
+          bad |= odd ? 1u << b : 0;
         }
+        bad_blocks[t & 1][16 * wave + (threadIdx.x & 15)] = (uint8_t)bad;
         asm volatile("" ::: "memory");
       }
       f32x16 s[2];
@@ -306,17 +309,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       if (!whole) {
         const Row q = my_row();
         const int pos = q.rho < rows ? rq.len - rq.n + q.token : INT32_MAX, first = q.rho < rows ? first_key(pos, a.window) : 0;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = k0 + 32 * kt + 16 * h + i;
-            if (key < first || key > pos) s[kt][i] = -__builtin_inff();
-          }
         const uint64_t seen = keys_between(first - k0, pos - k0);
 #pragma unroll
-        for (int d = 0; d < NB; ++d)
-          if (const uint64_t bad = *reinterpret_cast<const uint64_t *>(bad_keys[t & 1][d]); __any(bad != 0)) o[d] += bad & seen ? __builtin_nanf("") : 0.f;
+        for (int kt = 0; kt < 2; ++kt) {
+          const int mine = (int)(seen >> (32 * kt)) >> (16 * h);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {  // by bits: masks of lanes would take the scalar registers from the whole loop
+            const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe(mine, i, 1);
+            s[kt][i] = __uint_as_float((__float_as_uint(s[kt][i]) & keep) | (0xFF800000u & ~keep));
+          }
+        }
+        const uint32_t bad = bad_blocks[t & 1][lane];
+        if (__any(bad != 0)) {
+#pragma unroll 1
+          for (int d = 0; d < NB; ++d)
+            if (__ballot((bad >> d) & 1) & seen) taint |= 1u << d;
+        }
       }
       float mx = -__builtin_inff();
 #pragma unroll
@@ -386,6 +394,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     // ---- this lane's part of its row: dimensions 32 d + 8 i + 4 h and the next three
     const Row q = my_row();
     l = over_halves(l, [](float p, float q) { return p + q; });
+    if (__any(taint != 0)) {
+#pragma unroll
+      for (int d = 0; d < NB; ++d) o[d] += (taint >> d) & 1 ? __builtin_nanf("") : 0.f;
+    }
     if (q.rho < rows) {
       if (is_whole) {
         const float f = l == 0.f ? 0.f : 4.f / l;
