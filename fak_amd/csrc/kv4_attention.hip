@@ -648,17 +648,16 @@ int64_t steps_bound(const Attend &a) {
   return (seen + kStep - 1) / kStep;
 }
 
-// As many workgroups as stay resident on a CU (by the stages' LDS).
-constexpr int per_cu(int D, int waves) { return (D == 256 ? 4 : D == 64 ? 16 : 8) / waves; }
-
 template <int D, bool PACK, int kWaves>
 int run_split(const char *who, Attend a) {
   constexpr int RPT = PACK ? 8 : 16, kItemCost = item_cost(PACK), kLeast = least(PACK);
+  // As many workgroups as stay resident (by the stages' LDS).
+  constexpr int kPerCu = (D == 256 ? 4 : D == 64 ? 16 : 8) / kWaves;
   const int group = a.heads / a.heads_kv;
   const int64_t steps = (((int64_t)a.cols << a.shift) - 1) / kStep + 1;
   const int64_t row_tiles = ((int64_t)a.tokens * group) / RPT + a.requests;
   const int64_t most = std::min(row_tiles * a.heads_kv, (int64_t)1 << 31) * ((steps + kWaves - 1) / kWaves + kItemCost) / kLeast + 1;
-  const int grid = (int)std::min(std::min((int64_t)per_cu(D, kWaves) * cu_count(), (int64_t)kMostParts), most);
+  const int grid = (int)std::min(std::min((int64_t)kPerCu * cu_count(), (int64_t)kMostParts), most);
   // A request's items are bounded by the tokens that all requests have; where that bounds them all below the
   // grid, the joining launch is as large as that (28 rows of one long request: 32 workgroups, not 4,096).
   const int64_t per_request = ((int64_t)a.tokens * group + RPT - 1) / RPT * a.heads_kv;
@@ -683,24 +682,14 @@ int run_split(const char *who, Attend a) {
 }
 
 // Workgroups of four waves for single tokens of more items than CUs: an item's start and joins then keep half as
-// many waves from work. Eight and four waves, us, 8 key heads, all requests of one length:
-//   heads of 128  256 items of 128 keys 7.6 and 6.9, 500: 9.3 and 12.4, 2,000: 21 and 27
-//                 320                   11.2 and 8.4     14.7 and 12.7      31 and 30
-//                 1,024                 20.2 and 14.0    29.4 and 24.1      72 and 62
-//   heads of 64   256                   7.9 and 6.4      9.0 and 10.4       27 and 24
-//                 320                   11.5 and 7.4     14.0 and 10.4      30 and 25
-//                 512                   11.6 and 7.7     14.2 and 16.4      26 and 34
-//                 1,024                 19.3 and 13.7    24.0 and 18.3      47 and 41
-// and heads of 96 as of 128. So eight also where items nearly fill the places of such workgroups, once each (heads of
-// 64 have two to a CU), and tables allow more than four steps. (Tiles of 16 rows have no registers for four.)
+// many waves from work. One token of each of 1,000 requests of 100 keys, 28 heads over 4 of 128: 53 us, with eight
+// waves 86; 128 requests of 2,000 keys 35 and 42; but 64 requests of 500 keys, 256 items, 14 and 10. (Tiles of 16 rows
+// have no registers for it.)
 template <int D, bool PACK>
 int run_waves(const char *who, const Attend &a, int64_t rows) {
   constexpr int W = split_waves(D);
-  if constexpr (PACK && W == 8) {
-    const int64_t items = (rows + 7) / 8 * a.requests * a.heads_kv, places = (int64_t)per_cu(D, W) * cu_count();
-    const bool fill = items > places * 3 / 4 && items <= places && ((int64_t)a.cols << a.shift) > 4 * kStep;
-    if (items > cu_count() && !fill) return run_split<D, PACK, 4>(who, a);
-  }
+  if constexpr (PACK && W == 8)
+    if ((rows + 7) / 8 * a.requests * a.heads_kv > cu_count()) return run_split<D, PACK, 4>(who, a);
   return run_split<D, PACK, W>(who, a);
 }
 
