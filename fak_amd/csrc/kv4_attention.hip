@@ -682,9 +682,17 @@ int run_split(const char *who, Attend a) {
 }
 
 // Workgroups of four waves for single tokens of more items than CUs: an item's start and joins then keep half as
-// many waves from work. One token of each of 1,000 requests of 100 keys, 28 heads over 4 of 128: 53 us, with eight
-// waves 86; 128 requests of 2,000 keys 35 and 42; but 64 requests of 500 keys, 256 items, 14 and 10. (Tiles of 16 rows
-// have no registers for it.)
+// many waves from work. Eight and four waves, us, 8 key heads, all requests of one length:
+//   heads of 128  256 items of 128 keys 7.6 and 6.9, 500: 9.3 and 12.4, 2,000: 21 and 27
+//                 320                   11.2 and 8.4     14.7 and 12.7      31 and 30
+//                 1,024                 20.2 and 14.0    29.4 and 24.1      72 and 62
+//   heads of 64   256                   7.9 and 6.4      9.0 and 10.4       27 and 24
+//                 320                   11.5 and 7.4     14.0 and 10.4      30 and 25
+//                 512                   11.6 and 7.7     14.2 and 16.4      26 and 34
+//                 1,024                 19.3 and 13.7    24.0 and 18.3      47 and 41
+// and heads of 96 as of 128. What 512 items of heads of 64 lose, one for each place of an eight-wave workgroup, holds
+// for equal lengths alone: spread evenly over their logarithm up to 2,000 they take 25 and 17, up to 700 19 and 12.5.
+// (Tiles of 16 rows have no registers for four.)
 template <int D, bool PACK>
 int run_waves(const char *who, const Attend &a, int64_t rows) {
   constexpr int W = split_waves(D);
