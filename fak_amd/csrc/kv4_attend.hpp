@@ -113,6 +113,10 @@ __device__ inline Req request(const Attend &a, int begin, int end, int len) {
   return q;
 }
 
+// Whether the requests' first tokens fall here. Where none does, all requests have no more tokens than the call, and
+// their units stay below 2^31; else a launch takes none of them, since units past that would name items that are not.
+__device__ inline bool falling(const Attend &a, int r) { return a.start[r + 1] < a.start[r]; }
+
 // The inclusive sum over the lanes of a wave; the largest of them of numbers not below 0.
 #define FHIP_SCAN(f)                                                                                                          \
   f(0x111, 0xF) f(0x112, 0xF) f(0x114, 0xF) f(0x118, 0xF) /* rows of 16: shifts by 1, 2, 4, 8 */                              \

@@ -103,6 +103,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   static_assert(RPT * (OS + 2) <= STAGE, "a wave's results have to fit its stage");
   __shared__ u32x4 buf0[kWaves * STAGE / 4], buf1[kWaves * STAGE / 4];
   __shared__ int scan[kWaves], found_before, found_r;
+  __shared__ bool fallen[kWaves];
   __shared__ uint32_t is_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15, row = PACK ? col & 7 : col;
@@ -114,17 +115,25 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D =
   const bool few = a.requests <= 64;
   const int per = few ? 1 : (a.requests + kThreads - 1) / kThreads, r0 = min((few ? lane : tid) * per, a.requests), r1 = min(r0 + per, a.requests);
   int mine = 0, before, total;
+  bool falls = false;
   Req held;
   if (few) {
     held = load_request(min(r0, a.requests - 1));
     mine = r0 < a.requests ? held.units : 0;
+    falls = __any(r0 < a.requests && falling(a, r0));
     const int upto = sum_lanes(mine);
     before = upto - mine;
     total = __builtin_amdgcn_readlane(upto, 63);
   } else {
-    for (int r = r0; r < r1; ++r) mine += load_request(r).units;
+    for (int r = r0; r < r1; ++r) mine += load_request(r).units, falls |= falling(a, r);
+    falls = __any(falls);
+    if (lane == 0) fallen[wave] = falls;
     total = sum_before<kWaves>(mine, scan, &before);
+    falls = false;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) falls |= fallen[v];
   }
+  if (falls) total = 0, a.least_rows = INT64_MAX;
   const int G = total < (int)gridDim.x * kLeast ? max(total / kLeast, 1) : gridDim.x;
   // Neighbouring runs go to one XCD (blockIdx mod 8) and the row tiles of a kv head follow each other, so that
   // the tiles of many rows share their keys' lines in one L2: worth 2 to 3% (window of 1,024: 24.0 us, else 24.8 before the queries were shared).

@@ -46,6 +46,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   __shared__ u32x4 KF[64 * KU], VF[D * VU];
   __shared__ uint8_t bad_blocks[2][kStep];  // of each key of odd and even steps: a bit for each block
   __shared__ int scan_i[kWaves], scan_u[kWaves], found_before, found_r;
+  __shared__ bool fallen[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31, l16 = lane & 15, q4 = lane >> 4;
   const int group = a.heads / a.heads_kv, w = blockIdx.x;
@@ -54,13 +55,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   // ---- this workgroup's items, or its run of units
   const int per = (a.requests + kThreads - 1) / kThreads, r0 = min(tid * per, a.requests), r1 = min(r0 + per, a.requests);
   int my_items = 0, my_units = 0;
+  bool falls = false;
   for (int r = r0; r < r1; ++r) {
     const Req q = request<kRows, 1, kCost>(a, a.start[r], a.start[r + 1], a.lens[r]);
     my_items += q.row_tiles * a.heads_kv;
     my_units += q.units;
+    falls |= falling(a, r);
   }
+  falls = __any(falls);
+  if (lane == 0) fallen[wave] = falls;
   int before_i, before_u;
-  const int items = sum_before<kWaves>(my_items, scan_i, &before_i), units = sum_before<kWaves>(my_units, scan_u, &before_u);
+  int items = sum_before<kWaves>(my_items, scan_i, &before_i), units = sum_before<kWaves>(my_units, scan_u, &before_u);
+  if (fallen[0] || fallen[1] || fallen[2] || fallen[3]) items = units = 0;
   if (a.zero_rest) clear_rest(a, D);
   if (w < split_wgs && tid == 0) split[w].rows = 0;
   // 16 requests of 8,000 keys, 128 items: cut 150 us, whole 247; from 3/4 of the resident workgroups on, the joins

@@ -310,7 +310,7 @@ int fhip_kv4_read_f32(float *dK, float *dV, const void *dCache, const int32_t *d
  * of n stands at position p = dLens[r] - n + i and sees the keys max(0, p - window + 1) .. p (window 0:
  * no limit). dQ[t * ldq + head * head_dim + i], heads a multiple of heads_kv, each kv head serving
  * heads / heads_kv in a row; dOut[tokens][heads][head_dim]. A token without keys (p < 0, or past
- * dStart[requests]) gets zeros. dStart does not fall. max_new is at least every request's token count (it
+ * dStart[requests]) gets zeros. dStart begins at 0 and does not fall (a call whose does takes no request). max_new is at least every request's token count (it
  * only chooses between kernels, as does the number of positions a table row can hold; the plain decode step is 1:
  * a narrow table is the faster one for short requests). Lengths are clamped to the table row and page ids to the
  * cache, so no wrong table makes the call read outside it. All sums are f32 or wider over the cache's
