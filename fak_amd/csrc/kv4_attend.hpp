@@ -13,8 +13,10 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kStep = 64;   // keys of a wave's step: four granules
 constexpr double kLog2e = 1.44269504088896340736;
-// Weights are e^(..) 2^14: as f16 pairs they then keep 2^-38 of the largest, so that hundreds of
-// thousands of small ones add up right.
+// Weights are e^(..) 2^14: as two f16 terms they then keep 22 bits, and 2^-38 of the largest below, so that hundreds of
+// thousands of small ones add up right. Both terms are cut toward zero: where a score of 2^25 and more rounds the 14 to
+// 16, the first is f16's largest number and the second the rest, no infinity. (Terms for what two leave of the
+// smaller weights: prompts 330 us where they take 204, 32 single tokens 19 and 16.)
 constexpr float kBias = 14.f;
 
 struct Attend {
