@@ -19,7 +19,9 @@ the same names, argument meaning and failure behaviour (a Go panic becomes a Pyt
 * The backend class is Approx (harness-enforced, compute.go:212-217, 525).
 
 Only the quantized weight path lives here; RMSNorm/RoPE/attention and the f32/f16 GEMMs are
-outside this backend's scope and raise NotImplementedError.
+outside this backend's scope and raise NotImplementedError. (The serving entries, attention over the
+4-bit cache among them, have no counterpart in compute.Backend: they are called through fakhip, as
+serving_step.py does.)
 """
 from __future__ import annotations
 

@@ -7,9 +7,10 @@
 //
 // Bound by the matrix instructions: two terms of each f32 operand make 2 * 2 * 32 * 64 * 128 products of
 // a step, 2,048 of a SIMD's cycles, beside some 1,600 of vector instructions, which the CU's second
-// workgroup overlaps. Two prompts of 4,096 tokens, 2,048 of them new, 28 heads over 4 of 128: 205 to 230 us with
-// the card's clock, 182 GFLOP of products in two terms or 0.8 to 0.9 PFLOP/s, where a large f16 product reaches
-// 1.13; matrix and vector units are each busy a little over half of the time. In turn, not side by side, the same took 226.
+// workgroup overlaps. A chunk of 2,048 tokens behind 2,048 keys (beside one of ten tokens), 28 heads over 4 of 128: 190
+// to 225 us with the card's clock, 182 GFLOP of products in two terms or 0.8 to 0.95 PFLOP/s, where a large f16 product
+// reaches 1.13; matrix and vector units are each busy a little over half of the time. In turn, not side by side, the same
+// took 226. A fresh prompt of 4,096 tokens: 286 us, of 1,536 in cut items 93, since a cut counts the masked steps too.
 //
 // Items are whole where there are enough of them for the card; the steps of few long items are cut into
 // equal runs and joined by a second launch. Heads of 256 stay with the split kernel: 32 rows of them, two
