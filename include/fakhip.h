@@ -314,8 +314,9 @@ int fhip_kv4_read_f32(float *dK, float *dV, const void *dCache, const int32_t *d
  * only chooses between kernels, as does the number of positions a table row can hold; the plain decode step is 1:
  * a narrow table is the faster one for short requests). Lengths are clamped to the table row and page ids to the
  * cache, so no wrong table makes the call read outside it. All sums are f32 or wider over the cache's
- * exact values: within 1e-5 of the formula in the 2-norm; a weight below 2^-38 of its row's largest counts as
- * zero. scale is in (0, 1e37]. requests up to 65535. The steps of 64 keys that a table row allows, for each kv head
+ * exact values: within 1e-5 of the formula in the 2-norm. A weight is held to 2^-21 of itself or 2^-38 of its row's
+ * largest, whichever is more: one below that counts as zero, and an output that the larger weights all meet with values
+ * of 0 has the smaller ones' error. scale is in (0, 1e37]. requests up to 65535. The steps of 64 keys that a table row allows, for each kv head
  * and each 8 rows (tokens times heads / heads_kv; 16 or 128 rows where there are more), stay below about 2^31
  * for a batch's tokens, or the call is refused as too many. A NaN in a query makes its head's outputs
  * NaN, one in a key those of the rows that see it, one in a block of 32 values these 32 dimensions of them (an
