@@ -305,23 +305,24 @@ int fhip_kv4_append_f32(void *dCache, const float *dK, const float *dV, const in
  * outside it). */
 int fhip_kv4_read_f32(float *dK, float *dV, const void *dCache, const int32_t *dSlots, int tokens, int heads_kv,
                       int head_dim, int pages, int page);
-/* Attention of a batch over the 4-bit cache. Request r has dLens[r] keys (this batch's among them) in
- * the pages of dTable's row r, and the query tokens dStart[r] .. dStart[r+1]-1, its last ones: token i
- * of n stands at position p = dLens[r] - n + i and sees the keys max(0, p - window + 1) .. p (window 0:
- * no limit). dQ[t * ldq + head * head_dim + i], heads a multiple of heads_kv, each kv head serving
- * heads / heads_kv in a row; dOut[tokens][heads][head_dim]. A token without keys (p < 0, or past
- * dStart[requests]) gets zeros. dStart begins at 0 and does not fall (a call whose does takes no request). max_new is at least every request's token count (it
- * only chooses between kernels, as does the number of positions a table row can hold; the plain decode step is 1:
- * a narrow table is the faster one for short requests). Lengths are clamped to the table row and page ids to the
- * cache, so no wrong table makes the call read outside it. All sums are f32 or wider over the cache's
- * exact values: within 1e-5 of the formula in the 2-norm. A weight is held to 2^-21 of itself or 2^-38 of its row's
- * largest, whichever is more: one below that counts as zero, and an output that the larger weights all meet with values
- * of 0 has the smaller ones' error. scale is in (0, 1e37]. requests up to 65535. The steps of 64 keys that a table row allows, for each kv head
- * and each 8 rows (tokens times heads / heads_kv; 16 or 128 rows where there are more), stay below about 2^31
- * for a batch's tokens, or the call is refused as too many. A NaN in a query makes its head's outputs
- * NaN, one in a key those of the rows that see it, one in a block of 32 values these 32 dimensions of them (an
- * infinity the same); what lies behind a request's length is never seen. No counterpart in the
- * reference's device path (attention there reads an f32 cache, internal/compute/cuda_kernels.cu). */
+/* Attention of a batch over the 4-bit cache. Request r has dLens[r] keys (this batch's among them) in the pages of
+ * dTable's row r, and the query tokens dStart[r] .. dStart[r+1]-1, its last ones: token i of n stands at
+ * position p = dLens[r] - n + i and sees the keys max(0, p - window + 1) .. p (window 0: no limit). dQ[t * ldq
+ * + head * head_dim + i], heads a multiple of heads_kv, each kv head serving heads / heads_kv in a row;
+ * dOut[tokens][heads][head_dim]. A token without keys (p < 0, or past dStart[requests]) gets zeros. dStart
+ * begins at 0 and does not fall (a call whose does takes no request). max_new is at least every request's token
+ * count (it only chooses between kernels, as does the number of positions a table row can hold; the plain
+ * decode step is 1: a narrow table is the faster one for short requests). Lengths are clamped to the table row
+ * and page ids to the cache, so no wrong table makes the call read outside it. All sums are f32 or wider over
+ * the cache's exact values: within 1e-5 of the formula in the 2-norm. A weight is held to 2^-21 of itself or
+ * 2^-38 of its row's largest, whichever is more: one below that counts as zero, and an output that the larger
+ * weights all meet with values of 0 has the smaller ones' error. scale is in (0, 1e37]. requests up to 65535.
+ * The steps of 64 keys that a table row allows, for each kv head and each 8 rows (tokens times heads /
+ * heads_kv; 16 or 128 rows where there are more), stay below about 2^31 for a batch's tokens, or the call is
+ * refused as too many. A NaN in a query makes its head's outputs NaN, one in a key those of the rows that see
+ * it, one in a block of 32 values these 32 dimensions of them (an infinity the same); what lies behind a
+ * request's length is never seen. No counterpart in the reference's device path (attention there reads an f32
+ * cache, internal/compute/cuda_kernels.cu). */
 int fhip_kv4_attention_f32(const void *dCache, const float *dQ, float *dOut, const int32_t *dStart,
                            const int32_t *dLens, const int32_t *dTable, int requests, int tokens, int max_new,
                            int heads, int heads_kv, int head_dim, int pages, int page, int table_cols, int ldq,
